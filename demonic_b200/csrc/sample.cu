@@ -8,7 +8,8 @@
 // The k-th largest logit, or the one at which the mass reaches top_p, is found by histogram: 1024 bins over the distance
 // from the maximum (an order-preserving map, whatever its rounding) and the bin that holds the answer.  While no more
 // than 512 logits lie in the bins up to it, one CTA takes those, sorts them and finishes alone; else the bin's members are
-// ranked one against another, or split again while they are many, and the whole cluster goes on with the cut.
+// ranked one against another, or split again while they are many -- by the bits of the values, since different logits may lie
+// at one rounded distance -- and the whole cluster goes on with the cut.
 //
 // Measured on B200 (us a call): one row of 32000 f32 7 without a filter, 12 with top-k; 64 rows of 128000 f32 17 up to the maximum
 // (33 MB, 1.9 TB/s), 35 without a filter, 48 with top-k, 92 with top-p, 60 mixed; 256 rows of 50257 bf16 17 / 37 / 39 / 104.  Reading is the
@@ -34,7 +35,7 @@ namespace {
 // with four of 256).  Clusters of 16 were slower than 8 with larger slices (64 rows of 128000: 20 us against 15 up to the
 // maximum).
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 1024, kList = 512, kLevels = 6;
+constexpr int kBinBits = 10, kBins = 1 << kBinBits, kList = 512;
 constexpr int kMaxSlice = kSampleMaxVocab / kMaxCluster;  // logits of a row per CTA: 128 KiB of f32 at most
 constexpr double kOne = (double)(1ull << 44);    // mass of weight 1
 constexpr float kFar = 32.0f;                    // e^-32 * 2^44 rounds to 0
@@ -76,23 +77,24 @@ struct SampleSmem {
     u64 seg_mass[kMaxCluster];
     unsigned seg_count[kMaxCluster];
     Found found;
-    float near_d[kMaxCluster], far_d[kMaxCluster];  // extent of each CTA's members of a bin
+    unsigned least_key[kMaxCluster], most_key[kMaxCluster];  // extent of each CTA's members of a bin
     u64 part[kMaxCluster];
     u64 ws[16];
     unsigned wc[16];
     int n_list;                     // members of the bin, or of the leading bins, in this CTA
     u64 cut_key, cut_mass;
-    float red_f[16], red_g[16];
+    float red_f[16];
+    unsigned red_u[16], red_v[16];
     int red_i[16];
     int row;
 };
 
-// Greater value first, then lower index: a smaller key.
-__device__ __forceinline__ u64 key_of(float x, int i) {
+// Greater value first, then lower index: a smaller key.  Values are equal where their keys' high words are.
+__device__ __forceinline__ unsigned value_key(float x) {
     const unsigned u = __float_as_uint(x + 0.0f);  // (-0 orders as 0)
-    const unsigned ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((u64)~ord << 32) | (unsigned)i;
+    return (u & 0x80000000u) ? u : ~(u | 0x80000000u);
 }
+__device__ __forceinline__ u64 key_of(float x, int i) { return ((u64)value_key(x) << 32) | (unsigned)i; }
 __device__ __forceinline__ float value_of(u64 key) {
     const unsigned ord = ~(unsigned)(key >> 32);
     return __uint_as_float((ord & 0x80000000u) ? (ord & 0x7FFFFFFFu) : ~ord);
@@ -263,37 +265,31 @@ __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s
     const Cut limit = *cut;
     const int tid = threadIdx.x;
     const bool by_mass = q.need == 0;
-    // a member of level l's bin: floor((d - from[l]) * step[l]), limited to the last bin, == bin[l] for every earlier level
-    float from[kLevels], step[kLevels];
-    int bin[kLevels];
+    // Level 0 has its bins by distance; what is in the one it finds is binned by the value's key from then on, 10 bits of the
+    // members' extent at a time.  The map to bins is monotone at every level, so the members are the logits of an interval.
     u64 before = 0, inside = 0;
     unsigned count_before = 0, members = 0;
     double target = 0.0;
-    auto bin_of = [&](float d, int l) { return min(kBins - 1, (int)((d - from[l]) * step[l])); };
     const float step0 = (float)kBins / row.far;
-    int bin0 = 0;
-    auto member = [&](float x, int i, int levels) {
+    auto bin_of = [&](float d) { return min(kBins - 1, (int)(d * step0)); };
+    int bin0 = -1;                             // level 0's bin
+    unsigned from = 0, width = 0xFFFFFFFFu;    // keys from .. from + width, of which the bins have 2^shift each
+    int shift = 0, level = 0;
+    auto member = [&](float x, int i) {
         const float d = row.dist(x);
-        bool in = row.near(d) && limit.keeps(x, s.first + i);
-        if (levels > 0) in &= min(kBins - 1, (int)(d * step0)) == bin0;
-        for (int l = 1; l < levels; ++l) in &= bin_of(d, l) == bin[l];
-        return in;
+        return row.near(d) && limit.keeps(x, s.first + i) && (bin0 < 0 || bin_of(d) == bin0) && value_key(x) - from <= width;
     };
-    int level = 0;
-    from[0] = 0.0f;
-    step[0] = step0;
 #pragma unroll 1
     for (;; ++level) {
         for (int i = tid; i < kBins; i += TH) sm.h.count[i] = sm.h.lo[i] = sm.h.hi[i] = 0;
         __syncthreads();
         if (q.sparse) {
-            if (row.near(row.dist(own))) atomicAdd(&sm.h.count[bin_of(row.dist(own), 0)], 1u);
+            if (row.near(row.dist(own))) atomicAdd(&sm.h.count[bin_of(row.dist(own))], 1u);
         } else {
-            const float from_l = from[level], step_l = step[level];
             each(s, tid, s.n, TH, [&](float x, int i) {
                 const u64 m = by_mass ? row.mass(x) : 0;
-                if (!member(x, i, level)) return;
-                const int b = min(kBins - 1, (int)((row.dist(x) - from_l) * step_l));
+                if (!member(x, i)) return;
+                const int b = level == 0 ? bin_of(row.dist(x)) : (int)((value_key(x) - from) >> shift);
                 if (by_mass) {
                     const unsigned lo = (unsigned)m, was = atomicAdd(&sm.h.lo[b], lo);
                     const unsigned hi = (unsigned)(m >> 32) + (was + lo < was ? 1u : 0u);
@@ -353,43 +349,46 @@ __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s
         }
         cl.sync();
         const Found f = sm.found;
-        bin[level] = f.bin;
-        if (level == 0) bin0 = f.bin;
+        if (level == 0) {
+            bin0 = f.bin;
+        } else {
+            from += (unsigned)f.bin << shift;
+            width = min(width - ((unsigned)f.bin << shift), (1u << shift) - 1);  // (the last bin ends with its level)
+        }
         before = f.before, count_before = f.count_before, members = f.members, inside = f.inside;
         if (level == 0 && (q.sparse || count_before + members <= kList)) {
             *lead_bin = q.sparse && c_row < q.need ? kBins : f.bin;  // (fewer maxima than asked for say nothing)
             *lead_step = step0;
             return false;
         }
-        if (members <= kList || level + 1 == kLevels) break;
-        // many members: their own extent for the next level
-        float nd = INFINITY, fd = -INFINITY;
+        if (members <= kList) break;
+        // many members: their own extent for the next level.  It is less than 2^32 of keys at level 1 and than 2^10 times less
+        // at each further one, so level 5 would be one of equal values.
+        unsigned least = 0xFFFFFFFFu, most = 0;
         each(s, tid, s.n, TH, [&](float x, int i) {
-            if (member(x, i, level + 1)) nd = fminf(nd, row.dist(x)), fd = fmaxf(fd, row.dist(x));
+            if (member(x, i)) least = min(least, value_key(x)), most = max(most, value_key(x));
         });
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            nd = fminf(nd, __shfl_xor_sync(0xffffffffu, nd, o));
-            fd = fmaxf(fd, __shfl_xor_sync(0xffffffffu, fd, o));
-        }
-        if ((tid & 31) == 0) sm.red_f[tid >> 5] = nd, sm.red_g[tid >> 5] = fd;
+        least = __reduce_min_sync(0xffffffffu, least);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if ((tid & 31) == 0) sm.red_u[tid >> 5] = least, sm.red_v[tid >> 5] = most;
         __syncthreads();
-        for (int w = 0; w < TH / 32; ++w) nd = fminf(nd, sm.red_f[w]), fd = fmaxf(fd, sm.red_g[w]);
+        for (int w = 0; w < TH / 32; ++w) least = min(least, sm.red_u[w]), most = max(most, sm.red_v[w]);
         if (tid < s.ranks) {
-            cl.map_shared_rank(sm.near_d, tid)[s.rank] = nd;
-            cl.map_shared_rank(sm.far_d, tid)[s.rank] = fd;
+            cl.map_shared_rank(sm.least_key, tid)[s.rank] = least;
+            cl.map_shared_rank(sm.most_key, tid)[s.rank] = most;
         }
         cl.sync();
-        for (int r = 0; r < s.ranks; ++r) nd = fminf(nd, sm.near_d[r]), fd = fmaxf(fd, sm.far_d[r]);
-        if (nd == fd) break;  // all equal
-        from[level + 1] = nd;
-        step[level + 1] = (float)kBins / (fd - nd);
+        for (int r = 0; r < s.ranks; ++r) least = min(least, sm.least_key[r]), most = max(most, sm.most_key[r]);
+        if (least == most) break;  // all equal
+        from = least;
+        width = most - least;
+        shift = max(0, 32 - __clz((int)width) - kBinBits);
     }
     if (members <= kList) {  // the first CTA takes them, sorts them and tells the others
         if (tid == 0) sm.n_list = 0;
         __syncthreads();
         each(s, tid, s.n, TH, [&](float x, int i) {
-            if (member(x, i, level + 1)) sm.l.list[atomicAdd(&sm.n_list, 1)] = key_of(x, s.first + i);
+            if (member(x, i)) sm.l.list[atomicAdd(&sm.n_list, 1)] = key_of(x, s.first + i);
         });
         __syncthreads();
         int n;
@@ -421,13 +420,12 @@ __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s
         cl.sync();
         *cut = cut_of(sm.cut_key);
     } else {
-        // so many equal values: they are taken by index.  (All levels used up comes to the same: 1024^6 parts of a range
-        // of floats leave nothing to tell apart.)
+        // so many equal values: they are taken by index
         float x = 0.0f;
         unsigned c = 0;
         const int per = (s.n + TH - 1) / TH, i0 = min(s.n, tid * per), i1 = min(s.n, i0 + per);
         for (int i = i0; i < i1; ++i) {
-            if (member(s[i], i, level + 1)) {
+            if (member(s[i], i)) {
                 x = s[i];
                 ++c;
             }
@@ -456,7 +454,7 @@ __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s
             if (below + at < k && below + at + c >= k) {
                 unsigned j = below + at;
                 for (int i = i0; i < i1; ++i)
-                    if (member(s[i], i, level + 1) && ++j == k)
+                    if (member(s[i], i) && ++j == k)
                         for (int r = 0; r < s.ranks; ++r) *cl.map_shared_rank(&sm.cut_key, r) = key_of(s[i], s.first + i);
             }
         }

@@ -147,3 +147,35 @@ def test_batches_that_do_not_fit_at_once(batch, vocab, kind):
          "k_alone": None}[kind]
     t = np.where(rng.random(batch) < 0.1, 0.0, rng.uniform(0.5, 1.5, batch))
     check(x, t, k, p, None, rng.random(batch))
+
+
+def close_beside_a_large_one(kind, vocab, rng):
+    """One logit far above the rest, whose differences are lost in their distance from it (an f32)."""
+    if kind == "normal":
+        x = rng.standard_normal(vocab) * 1e-7
+    elif kind == "every size":                    # from 1e-8 down to below the smallest normal number, both signs, zeros
+        x = rng.choice([-1.0, 1.0], vocab) * 10.0 ** rng.uniform(-44, -8, vocab)
+        x[::50] = 0.0
+        x[1::50] = -0.0
+    else:                                         # neighbouring floats, each of them many times
+        x = np.float32(1e-6).view(np.int32) + rng.integers(0, 40, vocab).astype(np.int32)
+        x = x.view(F).astype(np.float64)
+    x[vocab // 3] = 20.0
+    return x.astype(F)
+
+
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["normal", "every size", "neighbours"])
+@pytest.mark.parametrize("t", [1.0, 10.0])
+@pytest.mark.parametrize("k,p", [(50, None), (600, None), (1000, None), (20000, None), (None, 0.3), (None, 0.9), (900, 0.6), (20000, 0.8)])
+def test_logits_closer_together_than_their_distance_from_the_largest(bf16, kind, t, k, p):
+    rng = np.random.default_rng(31)
+    x = close_beside_a_large_one(kind, 32000, rng)
+    bits = None
+    if bf16:
+        bits = f32_to_bf16_rne(x)
+        x = bf16_to_f32(bits).reshape(x.shape)
+    n = 12
+    rows = np.repeat(x[None], n, 0)
+    check(rows, np.full(n, t), None if k is None else [k] * n, None if p is None else [p] * n, None, (np.arange(n) + 0.5) / n,
+          bits=None if bits is None else np.repeat(bits.reshape(1, -1), n, 0))
