@@ -423,7 +423,7 @@ extern "C" int dmc_decoder_fork(void *dec, int src, int dst) {
     DMC_CUDA_TRY(cudaStreamSynchronize(ctx().stream));  // pair lives on this stack frame
     stream_drained();
     k->lens[dst] = k->lens[src];
-    if (k->lens[src] % k->cache.page_tokens) k->shared[src] = k->shared[dst] = 1;
+    if (k->lens[src]) k->shared[src] = k->shared[dst] = 1;  // (a full last page too: the benchmark writes into it again)
     return DMC_CUDA_OK;
 }
 

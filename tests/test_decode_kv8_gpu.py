@@ -167,3 +167,26 @@ def test_the_benchmark_writes_to_no_page_that_another_sequence_holds():
     assert np.array_equal(got, other.step(0, 6, want_logits=True)[2])
     other.close()
     dec.close()
+
+
+@pytest.mark.parametrize("held", [16, 32])
+@pytest.mark.parametrize("way", [(0, 1), (1, 0)], ids=["from", "to"])
+def test_the_benchmark_is_refused_where_a_full_last_page_is_shared(held, way):
+    model = decoder.random_model(CFG, seed=8, cache_len=0)
+    dec = decoder.Kv8Decoder(CFG, model, sequences=2, page_tokens=16)
+    for t in range(held):
+        dec.step(way[0], t)
+    dec.fork(*way)
+    with pytest.raises(_lib.DmcCudaError) as e:
+        dec.bench(999, held - 1, 1)             # would replace the last token of the page that both hold
+    assert e.value.code == 2 and "another sequence" in str(e.value)
+    _lib.load().dmc_cuda_clear_error()
+    dec.step(0, 6)                              # a page of its own
+    assert dec.bench(7, held, 1) > 0
+    got = dec.step(1, 6, want_logits=True)[2]
+    other = decoder.Kv8Decoder(CFG, model)
+    for t in range(held):
+        other.step(0, t)
+    assert np.array_equal(got, other.step(0, 6, want_logits=True)[2])
+    other.close()
+    dec.close()
