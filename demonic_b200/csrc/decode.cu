@@ -252,6 +252,25 @@ void free_kv8(Kv8State *k) {
     delete k;
 }
 
+// Everything that a decoder owns, its 8-bit cache included; one that was only partly allocated too.
+void free_decoder(Decoder *d) {
+    if (!d) return;
+    if (d->exec) cudaGraphExecDestroy(d->exec);
+    if (d->graph) cudaGraphDestroy(d->graph);
+    void *singles[] = {d->embed, d->lm_head, d->gf, d->rope_cos, d->rope_sin, d->h, d->xn, d->qkv, d->ao, d->d1, d->gu,
+                       d->act, d->d2, d->logits, d->part, d->d_token, d->d_pos, d->d_next, d->h2, d->attn_cnt, d->am_val, d->am_idx, d->am_cnt,
+                       d->am_key};
+    for (void *p : singles)
+        if (p) cudaFree(p);
+    for (Layer &L : d->layers) {
+        void *ps[] = {L.wqkv, L.wo, L.wgu, L.wd, L.g1, L.g2, L.kc, L.vc};
+        for (void *p : ps)
+            if (p) cudaFree(p);
+    }
+    free_kv8(d->kv8);
+    delete d;
+}
+
 int create_kv8(Kv8State &k, const dmc_decoder_config &cfg, int sequences, int64_t pages, int page_tokens) {
     dmc_kv8_cache &c = k.cache;
     dmc_kv8_seqs &q = k.seqs;
@@ -297,7 +316,7 @@ bool kv8_slot_ok(const Kv8State &k, int seq) { return seq >= 0 && seq < k.seqs.s
 
 using namespace dmc;
 
-static int create_decoder(const dmc_decoder_config *cfg, Kv8State *kv8, Decoder **out);
+static int create_decoder(const dmc_decoder_config *cfg, bool kv8, Decoder **out);
 
 extern "C" int dmc_decoder_create(const dmc_decoder_config *cfg, void **out) {
     std::lock_guard<std::mutex> lock(ctx_mutex());
@@ -308,16 +327,15 @@ extern "C" int dmc_decoder_create(const dmc_decoder_config *cfg, void **out) {
     int rc = ensure_init();
     if (rc) return rc;
     Decoder *d = nullptr;
-    if ((rc = create_decoder(cfg, nullptr, &d))) return rc;
+    if ((rc = create_decoder(cfg, false, &d))) return rc;
     *out = d;
     return DMC_CUDA_OK;
 }
 
-static int create_decoder(const dmc_decoder_config *cfg, Kv8State *kv8, Decoder **out) {
-    Decoder *d = new Decoder();
+// What every decoder has, and the f32 cache of one without an 8-bit cache.  The caller frees what a throw leaves in *d.
+static int alloc_decoder(const dmc_decoder_config *cfg, bool kv8, Decoder *d) {
     int rc;
     d->cfg = *cfg;
-    d->kv8 = kv8;
     const size_t D = cfg->d_model, F = cfg->ffn, V = cfg->vocab, H = cfg->heads, hd = cfg->head_dim, cap = cfg->max_len;
     d->layers.resize(cfg->layers);
     rc = dalloc(&d->embed, V * D) || dalloc(&d->lm_head, V * D) || dalloc(&d->gf, D) || dalloc(&d->rope_cos, cap * hd / 2) ||
@@ -330,9 +348,21 @@ static int create_decoder(const dmc_decoder_config *cfg, Kv8State *kv8, Decoder 
     for (Layer &L : d->layers)
         rc = rc || dalloc(&L.wqkv, 3 * D * D) || dalloc(&L.wo, D * D) || dalloc(&L.wgu, 2 * F * D) || dalloc(&L.wd, D * F) ||
              dalloc(&L.g1, D) || dalloc(&L.g2, D) || (!kv8 && (dalloc(&L.kc, H * cap * hd) || dalloc(&L.vc, H * cap * hd)));
-    if (rc) return dmc::status();
-    *out = d;
-    return DMC_CUDA_OK;
+    return rc ? dmc::status() : DMC_CUDA_OK;
+}
+
+static int create_decoder(const dmc_decoder_config *cfg, bool kv8, Decoder **out) {
+    Decoder *d = nullptr;
+    int rc;
+    try {
+        d = new Decoder();
+        rc = alloc_decoder(cfg, kv8, d);
+    } catch (const std::bad_alloc &) {  // not across the C boundary
+        rc = fail(DMC_CUDA_ERR_OOM, "decoder_create: host memory");
+    }
+    if (rc) free_decoder(d);
+    else *out = d;
+    return rc;
 }
 
 extern "C" int dmc_decoder_create_kv8(const dmc_decoder_config *cfg, int sequences, int64_t pages, int page_tokens, void **out) {
@@ -351,7 +381,7 @@ extern "C" int dmc_decoder_create_kv8(const dmc_decoder_config *cfg, int sequenc
     try {
         k = new Kv8State();
         rc = create_kv8(*k, *cfg, sequences, pages, page_tokens);
-        if (!rc) rc = create_decoder(cfg, k, &d);
+        if (!rc) rc = create_decoder(cfg, true, &d);
     } catch (const std::bad_alloc &) {  // not across the C boundary
         rc = fail(DMC_CUDA_ERR_OOM, "decoder_create_kv8: host memory");
     }
@@ -359,6 +389,7 @@ extern "C" int dmc_decoder_create_kv8(const dmc_decoder_config *cfg, int sequenc
         free_kv8(k);
         return rc;
     }
+    d->kv8 = k;
     *out = d;
     return DMC_CUDA_OK;
 }
@@ -587,18 +618,5 @@ extern "C" void dmc_decoder_destroy(void *dec) {
     Decoder *d = static_cast<Decoder *>(dec);
     if (!d) return;
     if (ctx().ready) cudaStreamSynchronize(ctx().stream);
-    if (d->exec) cudaGraphExecDestroy(d->exec);
-    if (d->graph) cudaGraphDestroy(d->graph);
-    void *singles[] = {d->embed, d->lm_head, d->gf, d->rope_cos, d->rope_sin, d->h, d->xn, d->qkv, d->ao, d->d1, d->gu,
-                       d->act, d->d2, d->logits, d->part, d->d_token, d->d_pos, d->d_next, d->h2, d->attn_cnt, d->am_val, d->am_idx, d->am_cnt,
-                       d->am_key};
-    for (void *p : singles)
-        if (p) cudaFree(p);
-    for (Layer &L : d->layers) {
-        void *ps[] = {L.wqkv, L.wo, L.wgu, L.wd, L.g1, L.g2, L.kc, L.vc};
-        for (void *p : ps)
-            if (p) cudaFree(p);
-    }
-    free_kv8(d->kv8);
-    delete d;
+    free_decoder(d);
 }

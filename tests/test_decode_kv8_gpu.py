@@ -1,4 +1,6 @@
 """The decode step over the 8-bit paged cache against a CPU restatement: decode_ref's step with the cache of kv8_ref."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -190,3 +192,26 @@ def test_the_benchmark_is_refused_where_a_full_last_page_is_shared(held, way):
     assert np.array_equal(got, other.step(0, 6, want_logits=True)[2])
     other.close()
     dec.close()
+
+
+@pytest.mark.parametrize("kv8", [True, False], ids=["kv8", "f32"])
+def test_a_decoder_that_does_not_fit_leaves_no_memory_behind(kv8):
+    lib, rt = _lib.load(), ctypes.CDLL("libcudart.so.12")
+    rt.cudaMemGetInfo.argtypes = [ctypes.POINTER(ctypes.c_size_t)] * 2
+    # embeddings of 128 MiB and activations of 3 GiB fit; the first layer's gate and up matrices, 256 GiB, do not
+    desc = _lib.DecoderConfig(2, 256, 2, 128, 1 << 28, 262144, 64, 1e-5)
+
+    def create():
+        out = ctypes.c_void_p()
+        rc = (lib.dmc_decoder_create_kv8(ctypes.byref(desc), 2, 64, 16, ctypes.byref(out)) if kv8
+              else lib.dmc_decoder_create(ctypes.byref(desc), ctypes.byref(out)))
+        assert rc == 4 and not out.value
+        lib.dmc_cuda_clear_error()
+        free, total = ctypes.c_size_t(), ctypes.c_size_t()
+        assert rt.cudaMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+        return free.value
+    first = create()                              # (the context and its first buffers are made on the way)
+    assert [create() for _ in range(3)] == [first] * 3
+    small = decoder.Kv8Decoder(CFG, decoder.random_model(CFG, seed=9, cache_len=0))
+    assert small.step(0, 3)[1] == 1.0
+    small.close()
