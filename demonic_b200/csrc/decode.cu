@@ -66,10 +66,11 @@ struct Decoder {
     int64_t launches_per_step = 0;
 };
 
+// Zeroed on the context's stream, which the first copies into it run on too: it does not wait for the default stream.
 template <typename T>
 int dalloc(T **p, size_t count) {
     DMC_CUDA_TRY(dmc_malloc((void **)p, count * sizeof(T)));
-    DMC_CUDA_TRY(cudaMemset(*p, 0, count * sizeof(T)));
+    DMC_CUDA_TRY(cudaMemsetAsync(*p, 0, count * sizeof(T), ctx().stream));
     return DMC_CUDA_OK;
 }
 

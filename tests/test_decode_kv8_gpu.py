@@ -215,3 +215,16 @@ def test_a_decoder_that_does_not_fit_leaves_no_memory_behind(kv8):
     small = decoder.Kv8Decoder(CFG, decoder.random_model(CFG, seed=9, cache_len=0))
     assert small.step(0, 3)[1] == 1.0
     small.close()
+
+
+def test_a_large_pool_starts_with_every_page_free():
+    """Zeroing 30 GiB takes milliseconds, in which the free stack is written already."""
+    pages = 1_900_000
+    dec = decoder.Kv8Decoder(CFG, decoder.random_model(CFG, seed=10, cache_len=0), sequences=2, pages=pages)
+    assert dec.free_pages == pages
+    for t in range(17):
+        dec.step(0, t)
+    assert dec.free_pages == pages - 2
+    dec.release(0)
+    assert dec.free_pages == pages
+    dec.close()
