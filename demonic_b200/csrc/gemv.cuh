@@ -79,6 +79,16 @@ __device__ __forceinline__ uint4 ldg_stream16(const void *p) {
     return v;
 }
 
+// The same for rows that a kernel before this one in the stream may have written: a coherent load, and one that stays behind
+// griddep_wait() (the form above is for data that nobody writes while the kernel lives, and may be moved).
+__device__ __forceinline__ uint4 ld_stream16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 // Programmatic dependent launch: everything before the wait (address setup and
 // the first weight loads, which no earlier kernel writes) overlaps the tail of
 // the previous kernel in the stream; x is only read after it.

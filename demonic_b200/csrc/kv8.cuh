@@ -82,18 +82,19 @@ __device__ __forceinline__ int kv8_scale_exp(float amax) {
 template <bool BF16>
 __device__ __forceinline__ float4 load_row4(const void *p, size_t at) {
     if constexpr (BF16) {
-        const uint2 w = __ldg((const uint2 *)((const uint16_t *)p + at));
+        const uint2 w = *(const uint2 *)((const uint16_t *)p + at);
         return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
                            __uint_as_float(w.y & 0xFFFF0000u));
     } else {
-        return __ldg((const float4 *)((const float *)p + at));
+        return *(const float4 *)((const float *)p + at);
     }
 }
 
-// 16 bytes of a row: 8 bf16 or 4 f32.
+// 16 bytes of a row: 8 bf16 or 4 f32.  (A plain load: the kernel before may have written the row, so it must not be a read-only
+// one, which would take 17.2 us instead of 17.4 for the prompt below; streaming forms took 17.7.)
 template <bool BF16>
 __device__ __forceinline__ uint4 load_row16(const void *p, size_t at, bool vec) {
-    if (vec) return ldg_stream16((const char *)p + at * (BF16 ? 2 : 4));
+    if (vec) return *(const uint4 *)((const char *)p + at * (BF16 ? 2 : 4));
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -111,11 +112,11 @@ __device__ __forceinline__ uint4 load_row16(const void *p, size_t at, bool vec) 
 // registers, their maximum decides the scale, the codes go out.  A thread holds VPT pieces of 16 bytes.
 //   few tokens   a warp each (NTHR = 32): nothing to wait for but its own lanes
 //   prompts      256 threads each, a whole page in registers (16 of them for bf16, so that eight CTAs run on an SM)
-// Prompts are bound by HBM: 3 x 4001 tokens x 8 heads x 128, K and V bf16, 74 MB in 16.5 us = 4.5 TB/s; converting to f32 on
+// Prompts are bound by HBM: 3 x 4001 tokens x 8 heads x 128, K and V bf16, 74 MB in 17.4 us = 4.2 TB/s; converting to f32 on
 // arrival (32 registers, four CTAs) took 42.  A batch's single tokens are bound by latency (length -> page -> scale): 7 us.
 template <int HD, int NTHR, int VPT, bool BF16>
-__global__ void __launch_bounds__(256, NTHR == 256 && BF16 ? 8 : 4) kv8_append_kernel(Kv8Layer c, Kv8Rows r, const void *__restrict__ kx,
-                                                                                    const void *__restrict__ vx, long long row_stride,
+__global__ void __launch_bounds__(256, NTHR == 256 && BF16 ? 8 : 4) kv8_append_kernel(Kv8Layer c, Kv8Rows r, const void *kx,
+                                                                                    const void *vx, long long row_stride,
                                                                                     int touch, int vec) {
     constexpr int PER = 256 / NTHR, E = BF16 ? 8 : 4, PIECES = HD / E;
     __shared__ float red[8];

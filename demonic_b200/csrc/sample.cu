@@ -548,11 +548,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_kernel(SampleArgs a) {
     for (; v + 3 * TH < nv; v += 4 * TH) {
         uint4 w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = ldg_stream16(gv + v + j * TH);
+        for (int j = 0; j < 4; ++j) w[j] = ld_stream16(gv + v + j * TH);
 #pragma unroll
         for (int j = 0; j < 4; ++j) put(v + j * TH, w[j]);
     }
-    for (; v < nv; v += TH) put(v, ldg_stream16(gv + v));
+    for (; v < nv; v += TH) put(v, ld_stream16(gv + v));
     auto rewrite = [&](auto f) {
         for (int i = tid; i < s.n; i += TH) {
             const float y = f(s[i]);
