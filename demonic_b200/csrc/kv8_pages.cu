@@ -257,7 +257,8 @@ __global__ void __launch_bounds__(kThreads) kv8_release_kernel(PageArgs a) {
     auto page_at = [&](long long e) -> int {  // page that entry e gives back, or -1
         const int i = (int)(e / a.table_stride), s = a.ids[i];
         if (s < 0 || s >= a.slots || first[s] != i) return -1;
-        if ((int)(e % a.table_stride) >= held_pages(a, a.lens[s])) return -1;
+        const int n = a.lens[s];
+        if (n > a.cap || (int)(e % a.table_stride) >= held_pages(a, n)) return -1;
         const int p = a.table[(size_t)s * a.table_stride + e % a.table_stride];
         if ((unsigned)p < (unsigned)a.pages) return p;
         atomicOr(a.flags, DMC_KV8_BAD_PAGE);
@@ -266,6 +267,7 @@ __global__ void __launch_bounds__(kThreads) kv8_release_kernel(PageArgs a) {
     for (int i = rank * kThreads + threadIdx.x; i < a.count; i += kCluster * kThreads) {
         const int s = a.ids[i];
         if (s < -1 || s >= a.slots || (s >= 0 && first[s] != i)) atomicOr(a.flags, DMC_KV8_BAD_SLOT);
+        else if (s >= 0 && a.lens[s] > a.cap) atomicOr(a.flags, DMC_KV8_TOO_LONG);
     }
     for (long long e = e0 + threadIdx.x; e < e1; e += kThreads) {
         const int p = page_at(e);
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) kv8_release_kernel(PageArgs a) {
     cl.sync();  // every length has been read
     for (int i = rank * kThreads + threadIdx.x; i < a.count; i += kCluster * kThreads) {
         const int s = a.ids[i];
-        if (s >= 0 && s < a.slots) a.lens[s] = 0;
+        if (s >= 0 && s < a.slots && a.lens[s] <= a.cap) a.lens[s] = 0;
     }
     if (rank == 0 && threadIdx.x == 0) *a.free_count = min(fc + all, a.pages);
 }
@@ -359,8 +361,9 @@ __global__ void __launch_bounds__(kThreads) kv8_compact_kernel(PageArgs a) {
     cl.sync();
     const long long entries = (long long)a.slots * a.table_stride;
     for (long long e = gid; e < entries; e += kCluster * kThreads) {
-        const int s = (int)(e / a.table_stride);
-        if ((int)(e % a.table_stride) >= held_pages(a, a.lens[s])) continue;
+        const int s = (int)(e / a.table_stride), col = (int)(e % a.table_stride), n = a.lens[s];
+        if (n > a.cap && col == 0) atomicOr(a.flags, DMC_KV8_TOO_LONG);  // (renamed as far as it goes: its pages move too)
+        if (col >= held_pages(a, n)) continue;
         const int p = a.table[e];
         if ((unsigned)p < (unsigned)a.pages) a.table[e] = __ldcg(&page_map(a)[p]);
         else atomicOr(a.flags, DMC_KV8_BAD_PAGE);

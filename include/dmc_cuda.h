@@ -400,9 +400,9 @@ void dmc_decoder_destroy(void *dec);
  * (after dmc_cuda_init).  Pointers that are not device memory of that device are refused.  Calls on one
  * dmc_kv8_seqs change it and have to be ordered on one stream (or by events).
  *
- * What the host cannot see -- a slot or page id out of range, an empty pool -- the kernels check: the
- * row concerned (or the whole call, for dmc_kv8_reserve) is left out and a bit is set in *seqs.flags, which
- * the caller clears.  */
+ * What the host cannot see -- a slot or page id out of range, a length that its row cannot hold, an empty pool -- the
+ * kernels check: the row concerned (or the whole call, for dmc_kv8_reserve) is left out and a bit is set in
+ * *seqs.flags, which the caller clears.  (dmc_kv8_compact renames all pages that a row too long names, and sets the bit.)  */
 typedef struct dmc_kv8_cache {
     void *k, *v;              /* codes [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned        */
     float *k_scale, *v_scale; /* [layers][pages][kv_heads]; a key is code * scale.  Finite, in [2^-40, 2^40] or 0 */
