@@ -246,7 +246,7 @@ __device__ __forceinline__ int share_count(SampleSmem &sm, cg::cluster_group &cl
 }
 
 // What is asked of a row: its shortest leading part, in order (value down, index up), that has at least `need` members, or
-// (need == 0) at least `part` of the mass `of` (of the row's own, if that is 0).
+// (need == 0) at least `part` of the mass of what is kept so far, which leading_part leaves in `of`.
 struct Query {
     unsigned need;
     double part;
@@ -261,7 +261,7 @@ template <int TH, bool BF16>
 __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s, const Row row, float own, Query &query, Cut *cut,
                                           int *lead_bin, float *lead_step) {
     cg::cluster_group cl = cg::this_cluster();
-    Query q = query;
+    const Query q = query;
     const Cut limit = *cut;
     const int tid = threadIdx.x;
     const bool by_mass = q.need == 0;
@@ -334,8 +334,8 @@ __device__ __forceinline__ bool leading_part(SampleSmem &sm, const Slice<BF16> s
         }
         mb += m_at, cb += c_at;
         if (level == 0 && by_mass) {
-            if (q.of == 0) query.of = q.of = m_row;
-            target = fmax(q.part * (double)q.of, 1.0);
+            query.of = m_row;
+            target = fmax(q.part * (double)m_row, 1.0);
         }
         // (asked for more than there is: the last member is the answer)
         const unsigned want = min(q.need, c_row);
@@ -628,18 +628,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH) sample_kernel(SampleArgs a) {
         if (a.prob) a.prob[r] = (float)(row.scaled(value) / (double)total);
     };
 
-    u64 of = 0;  // the mass that top_p is a part of, once it is known
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         // 0: the k-th largest by way of the threads' maxima, while k is small among them; 1: the same by all; 2: top_p
         if (pass == 0 ? !by_k || !few(k, s.ranks * TH) : pass == 1 ? !by_k : !by_p) continue;
-        Query q{pass < 2 ? (unsigned)k : 0u, (double)p, of, pass == 0};
+        Query q{pass < 2 ? (unsigned)k : 0u, (double)p, 0, pass == 0};
         int lead_bin;
         float lead_step;
-        if (leading_part<TH>(sm, s, row, own, q, &cut, &lead_bin, &lead_step)) {
-            if (pass == 1) of = 0;
-            continue;
-        }
+        if (leading_part<TH>(sm, s, row, own, q, &cut, &lead_bin, &lead_step)) continue;
         // few logits lead: the first CTA takes them all and finishes
         if (tid == 0) sm.n_list = 0;
         __syncthreads();
