@@ -108,8 +108,8 @@ struct Row {
     __device__ __forceinline__ bool near(float d) const { return d <= far; }
     // 2^44 w for a near x.  16 (x - top) log2(e) / T = 16 n + j + r with |r| <= 1 / 2; 2^(r / 16) by a polynomial of degree 4
     // through the Chebyshev points of that interval (2^-38 off at most), 2^(j / 16) from the table, n into the exponent.
-    // b is off by half a unit of its last place, 2^-34 while |top| log2(e) / T is below 2^16 (the kernel sees to that): all
-    // weights of the row share that factor.
+    // b is off by half a unit of its last place, 2^-34 while |top| log2(e) / T is below 2^16 (the kernel sees to that): a
+    // factor of 2^(2^-34 / 16), less than 1 + 2^-38, which all weights of the row share.
     __device__ __forceinline__ double scaled(float x) const {
         const double y = fma((double)x, c, b);
         const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low word

@@ -497,8 +497,9 @@ int dmc_kv8_copy_pages(const dmc_kv8_cache *cache, const dmc_kv8_seqs *seqs, con
  * Arrays of one value per row, on the device; NULL stands for temperature 1, and for no filter, NaN for no filter.  A temperature that is
  * not above 0 takes the first maximum.  u is in [0, 1).  A NaN logit counts as -inf; a row of nothing else gives token -1
  * and probability 0.  tokens[batch]; prob (or NULL) [batch]: the token's probability in the distribution it was drawn from.
- * Sums are of integers, w_i * 2^44 rounded (the weights of a row share a factor that is off by 2^-33 at most), so the result
- * does not depend on the order of summation.
+ * Sums are of integers, w_i * 2^44 rounded (w_i is off by 2^-38 of itself at most, apart from a factor within 2^-38 of 1 that
+ * all weights of a row share), so the result does not depend on the order of summation.  A logit further below the maximum
+ * than the largest f32 counts as -inf.
  * vocab <= 262144.  No workspace; calls may run at the same time. */
 int dmc_cuda_sample(const void *logits, int xdtype, int64_t batch, int64_t vocab, int64_t row_stride, const float *temperature,
                     const int *top_k, const float *top_p, const float *min_p, const float *u, int *tokens, float *prob,
