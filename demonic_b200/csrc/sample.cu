@@ -772,8 +772,11 @@ int launch_sample(const void *logits, int xdtype, int64_t batch, int64_t vocab, 
     a.slice = (int)((vocab + cluster - 1) / cluster + 7) / 8 * 8;
     const int threads = a.slice <= few ? 256 : 512;
     // More clusters than fit at once: the slow rows first, lest one of them begins last (64 rows of 128000, filters mixed: 71 us
-    // in order, 60 so; looking at the filters costs 2 us where none is set: 256 rows of 50257 35 us in order, 37 so).
-    const int64_t at_once = (int64_t)ctx().sm_count * (1024 / threads) / cluster;
+    // in order, 60 so; 24 rows of 262144 f32, of which one slice fills an SM: 59 and 46; looking at the filters costs 2 us where
+    // none is set: 256 rows of 50257 35 us in order, 37 so).  By registers 1024 threads fit on an SM, by shared memory (228 KiB,
+    // of which each CTA takes 1 KiB more than it asks for) fewer once an f32 slice is above 100 KiB.
+    const int64_t per_sm = std::min<int64_t>(1024 / threads, (228 << 10) / (int64_t)(sample_smem(a.slice, bf16) + 1024));
+    const int64_t at_once = ctx().sm_count * per_sm / cluster;
     a.batch = batch > at_once && batch <= kRowsEach * threads && (top_k || top_p) ? (int)batch : 0;
     const void *fn = threads == 256 ? (bf16 ? (const void *)sample_kernel<256, true> : (const void *)sample_kernel<256, false>)
                                     : (bf16 ? (const void *)sample_kernel<512, true> : (const void *)sample_kernel<512, false>);

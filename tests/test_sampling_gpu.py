@@ -179,3 +179,12 @@ def test_logits_closer_together_than_their_distance_from_the_largest(bf16, kind,
     rows = np.repeat(x[None], n, 0)
     check(rows, np.full(n, t), None if k is None else [k] * n, None if p is None else [p] * n, None, (np.arange(n) + 0.5) / n,
           bits=None if bits is None else np.repeat(bits.reshape(1, -1), n, 0))
+
+
+def test_largest_rows_that_do_not_fit_at_once():
+    """An f32 slice of 128 KiB fills an SM, so that 19 rows and more are taken in the order of their cost."""
+    rng = np.random.default_rng(77)
+    batch, vocab = 21, 262144
+    x = (rng.standard_normal((batch, vocab)) * 2).astype(F)
+    i = np.arange(batch)
+    check(x, np.full(batch, 0.8), np.where(i % 3 == 1, 50, 0), np.where(i % 3 == 2, 0.9, 1.0), None, rng.random(batch))
