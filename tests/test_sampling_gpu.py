@@ -188,3 +188,16 @@ def test_largest_rows_that_do_not_fit_at_once():
     x = (rng.standard_normal((batch, vocab)) * 2).astype(F)
     i = np.arange(batch)
     check(x, np.full(batch, 0.8), np.where(i % 3 == 1, 50, 0), np.where(i % 3 == 2, 0.9, 1.0), None, rng.random(batch))
+
+
+def test_a_logit_beyond_the_range_of_f32_below_the_largest_is_never_drawn():
+    x = np.full((4, 100), -3e38, F)
+    x[:, 7] = 3e38
+    for k, p in ((None, None), ([5] * 4, None), (None, [0.9] * 4)):
+        u, tokens, prob = DeviceBuffer.from_host(np.array([0, .4, .9, .999], F)), DeviceBuffer(16), DeviceBuffer(16)
+        dev = {n: None if a is None else DeviceBuffer.from_host(np.asarray(a, np.int32 if n == "top_k" else F))
+               for n, a in (("top_k", k), ("top_p", p))}
+        sampling.sample(DeviceBuffer.from_host(x), 4, 100, tokens, u, temperature=DeviceBuffer.from_host(np.full(4, np.inf, F)),
+                        prob=prob, **dev)
+        backend.sync()
+        assert tokens.download(np.int32, 4).tolist() == [7] * 4 and prob.download(F, 4).tolist() == [1.0] * 4
