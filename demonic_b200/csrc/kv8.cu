@@ -98,7 +98,7 @@ const void *attn_fn(int hd, int nt, bool bf16, bool cluster, size_t *smem) {
 AttnPlan plan_attention(int hd, int hk, int q_heads, int batch, int tokens, int sms) {
     AttnPlan p;
     const int rows = tokens * (q_heads / hk);
-    // 8 rows per tile, or as many as the registers carry: a second tile reads the keys again
+    // 8 rows per tile, or as many as the registers carry: a second tile reads the keys again (what that costs: kv8.cuh)
     p.nt = std::min((rows + 7) / 8, hd == 128 ? 2 : 4);
     p.row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
     const int per_sm = hd == 128 ? Kv8Ring<128>::ctas_per_sm(p.nt) : Kv8Ring<64>::ctas_per_sm(p.nt);

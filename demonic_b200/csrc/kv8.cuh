@@ -112,8 +112,10 @@ __device__ __forceinline__ uint4 load_row16(const void *p, size_t at, bool vec) 
 // registers, their maximum decides the scale, the codes go out.  A thread holds VPT pieces of 16 bytes.
 //   few tokens   a warp each (NTHR = 32): nothing to wait for but its own lanes
 //   prompts      256 threads each, a whole page in registers (16 of them for bf16, so that eight CTAs run on an SM)
-// Prompts are bound by HBM: 3 x 4001 tokens x 8 heads x 128, K and V bf16, 74 MB in 17.4 us = 4.2 TB/s; converting to f32 on
-// arrival (32 registers, four CTAs) took 42.  A batch's single tokens are bound by latency (length -> page -> scale): 7 us.
+// Prompts are bound by issue: 3 x 4001 tokens x 8 heads x 128, K and V bf16, 74 MB in 17.4 us = 4.2 TB/s, issue slots 79 % and ALU
+// 53 % busy with scaling, converting and packing; f32 123 MB in 24.0 us = 5.1 TB/s.  Converting bf16 to f32 on arrival (32 registers,
+// four CTAs) took 42.  At the 32 registers that eight CTAs leave, the bf16 builds spill 56 (head_dim 128) and 28 bytes.  A batch's
+// single tokens are bound by latency (length -> page -> scale): 7 us.
 template <int HD, int NTHR, int VPT, bool BF16>
 __global__ void __launch_bounds__(256, NTHR == 256 && BF16 ? 8 : 4) kv8_append_kernel(Kv8Layer c, Kv8Rows r, const void *kx,
                                                                                     const void *vx, long long row_stride,
@@ -234,8 +236,8 @@ __global__ void __launch_bounds__(256, NTHR == 256 && BF16 ? 8 : 4) kv8_append_k
 // S' = K . Q' and O' = V' . P' on the tensor cores by mma.sync, keys (then dims) as the 16 rows and up to 8 query rows
 // (tokens x heads of the group) as the 8 columns, so that a group of 8 heads wastes nothing and a warp takes each code once.
 // (tcgen05 would need 128 rows of one operand and both in one type; here one side is 8 wide and the kernel is bound by memory.
-// m16n8k32 on the codes themselves is no way out: on this part it runs as conversions to f16 and two f16 products, measured at
-// 0.23 a clock and SM with new operands against 0.47 for m16n8k16.)  The codes are converted to f16, which is exact; f32 q and
+// m16n8k32 on the codes themselves is no way out: it was measured at 0.23 a clock and SM with new operands, against 0.47 for
+// m16n8k16.)  The codes are converted to f16, which is exact; f32 q and
 // probabilities enter as two f16 terms each (22 bits), bf16 q as one, which holds it exactly down to 2^-22 of the row's
 // largest element, and its probabilities as one (11 bits).
 //
@@ -245,11 +247,15 @@ __global__ void __launch_bounds__(256, NTHR == 256 && BF16 ? 8 : 4) kv8_append_k
 // of its V scale joins the score's, so that probabilities times V scale stay in range whatever the scales are, and the
 // rest (1 for a power of two) multiplies the probability.
 //
-// Bound by HBM for bf16 and few rows: 64 sequences of 8001-16000 keys x 8 heads, 8 query heads each, 1.58 GB in 258 us = 6.13
-// TB/s (0.94 of a plain copy's rate); the copies alone, without a product, took 255.  One sequence of 200001 keys x 4 heads: 47 us
-// for 205 MB, of which 5 the join and 4 the way to the first key.  f32 rows are bound by issue and
+// Bound by HBM for few rows: 64 sequences of 8001-16000 keys x 8 heads, 8 query heads each, 1.58 GB in 254-266 us = 6.0-6.2
+// TB/s (0.91-0.95 of a plain copy's rate); the copies alone, without a product, took 255.  One sequence of 200001 keys x 4 heads: 47 us
+// for 205 MB, of which 5 the join and 4 the way to the first key.  Many f32 rows are bound by issue and
 // latency: 5 tokens x 4 heads as two f16 terms each, over 400 warp instructions per 16 keys x 64 dims, issue slots 43 % and
-// the tensor pipe 37 % busy with the 12 warps that the registers allow, 62 us for 117 MB.
+// the tensor pipe 38 % busy with the 11 warps that the registers allow, 62 us for 117 MB.
+//
+// A tile's rows are as many as one warp's registers carry (16, or 32 of head_dim 64; the widest builds spill 24 to 68 bytes), and each
+// further tile of a head reads its keys again: 2 tokens of the 64 sequences above (16 rows) take 254 us in bf16 and 350 in f32, 5
+// tokens (40 rows, three tiles) 714 and 998.  A bf16 prompt of 1000 tokens, 32 heads over 8 x 128, takes 135 us, one of 4001 1330.
 constexpr int kKv8Warps = 4, kKv8MaxCluster = 8;
 constexpr int kKv8Unit = 16 * kKv8Warps;  // keys that a CTA takes at a time, 16 to a warp
 constexpr int kKv8Batch = 16;             // tiles of 16 keys whose places a warp looks up together

@@ -5,7 +5,7 @@
 // another: one CTA (reserve) or one cluster of 8 CTAs whose steps are separated by cluster barriers, never the whole
 // device.  What moves bytes is one copy kernel over a list of (source, destination) that the bookkeeping leaves in the
 // scratch area: 250 pages of 8 layers, 262 MB both ways, in 43 us = 6.1 TB/s (0.93 of a plain copy's rate).  The bookkeeping is
-// bound by latency, about 1 us per dependent load or barrier: fork 7 us (56 slots), reserve 8 (64 slots), compact 10 (1000 pages).
+// bound by latency, barriers the longest stall by far: fork 7 us (56 slots), reserve 9 (64 slots), compact 11 (1000 pages).
 #include <cooperative_groups.h>
 
 #include <algorithm>

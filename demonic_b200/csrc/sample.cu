@@ -11,10 +11,12 @@
 // ranked one against another, or split again while they are many -- by the bits of the values, since different logits may lie
 // at one rounded distance -- and the whole cluster goes on with the cut.
 //
-// Measured on B200 (us a call): one row of 32000 f32 7 without a filter, 12 with top-k; 64 rows of 128000 f32 17 up to the maximum
-// (33 MB, 1.9 TB/s), 35 without a filter, 48 with top-k, 92 with top-p, 60 mixed; 256 rows of 50257 bf16 17 / 37 / 39 / 104.  Reading is the
-// smaller part: 11 double operations and about 20 others per weight, atomics on random bins for top-p, and 2 us for every barrier
-// of a cluster.
+// Measured on B200 (us a call): one row of 32000 f32 5.4 for the maximum alone, 7 without a filter, 12 with top-k, 25 with top-p;
+// 64 rows of 128000 f32 15 (33 MB, 2.1 TB/s) / 31 / 44 / 83, 55 mixed; 256 rows of 50257 bf16 16 / 35 / 37 / 112.  No unit is full: in
+// the last case without a filter issue slots are 58 % busy, ALU 34 %, FP64 25 %, HBM 8 %, 26 warps per SM; with mixed filters 47 %,
+// 30 %, 7 %, 7 %, and barriers the longest stall.  A cluster loads its row, then works on it: while it does the one it does not do
+// the other, and 256 rows are 1.8 times what runs at once.  One row is latency: barriers of its cluster, and steps of one CTA.
+// At 64 registers the builds spill 8 (512 threads) and 32 bytes (256).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -30,10 +32,13 @@ namespace cg = cooperative_groups;
 namespace dmc {
 namespace {
 
-// CTAs of 256 threads while a slice is at most 28 KiB, else of 512: 1024 threads per SM either way (64 registers each), but four
-// CTAs in different phases hide one another's barriers (256 rows of 50257 bf16 logits: 57 us with two CTAs of 512 threads, 35
-// with four of 256).  Clusters of 16 were slower than 8 with larger slices (64 rows of 128000: 20 us against 15 up to the
-// maximum).
+// CTAs of 256 threads while a slice is at most 28 KiB, else of 512: 1024 threads per SM either way (64 registers each, while
+// shared memory holds so many slices), but four CTAs in different phases hide one another's barriers (256 rows of 50257 bf16
+// logits, 25 KiB: 57 us with two CTAs of 512 threads, 35 with four of 256).  From 28 to 43 KiB four CTAs fit as well, and which is
+// better goes by the rows: 64 of 128256 bf16 (31 KiB) 31 us with 512 threads and 23 with 256 without a filter, 54 and 58 mixed; 256
+// of them 106 and 72, 184 and 127 mixed; but 16 of them 38 and 52 with top-p, since the longest row then counts; 64 of 80000 f32
+// (39 KiB) 25 and 20, 47 and 51 mixed.  Clusters of 16 were slower than 8 with larger slices (64 rows of 128000: 20 us against 15
+// up to the maximum).
 constexpr int kMaxCluster = 8;
 constexpr int kBinBits = 10, kBins = 1 << kBinBits, kList = 512;
 constexpr int kMaxSlice = kSampleMaxVocab / kMaxCluster;  // logits of a row per CTA: 128 KiB of f32 at most
